@@ -14,7 +14,6 @@ Three operators of the transformer block around the INT8 linear layers:
 ``run`` computes their plain forms from elementary torch operations, or calls the
 framework where ``own`` is true.
 """
-import functools
 import math
 import random
 import sys
@@ -307,7 +306,6 @@ def _plain_attn(s):
 _PLAIN = {"rms": _plain_rms, "rope": _plain_rope, "table": _plain_table, "attn": _plain_attn}
 
 
-@functools.cache
 def _framework():
     path = str(Path(__file__).resolve().parents[1] / "comfyui-h3-speedkit_b200")
     if path not in sys.path:
@@ -320,9 +318,7 @@ def _own_rms(s):
     codes, scale, h = _framework()[1].residual_rms_quant(
         s["x"], s["weight"], residual=s["residual"], eps=EPS,
         dtype=torch.int8 if s["case"]["codes"] == "int8" else torch.float8_e4m3fn)
-    # what the codes stand for, in one pass (eight-bit floats are exact in either type)
-    codes = codes if codes.dtype == torch.int8 else codes.to(s["x"].dtype)
-    return {"values": torch.mul(codes, scale, out=torch.empty_like(s["x"])), "scale": scale, "sum": h}
+    return {"values": (codes.float() * scale).to(s["x"].dtype), "scale": scale, "sum": h}
 
 
 def _own_rope(s):
