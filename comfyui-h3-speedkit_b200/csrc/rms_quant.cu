@@ -10,9 +10,13 @@
 // max|y| = max|h w| * rstd exactly (rounding is monotone).  The codes are
 // (h w) * (rstd / s), one multiplication each.  HBM bound: 2 K (+ 2 K with a
 // residual) bytes in, K (+ 2 K) + 4 out per row.  16384 rows of 5376, BF16 with a residual:
-// 100 us, 6.14 TB/s, 0.94 of a copy's; one row of 4096 4.1 us, most of it the launch.
+// 96.4 us, 6.40 TB/s, 0.98 of a copy's; one row of 4096 4.1 us, most of it the launch.
 //
-// A row whose values are not all finite gets a NaN scale; other rows are
+// That form holds where its numbers are in FP32's range (`ordinary`).  Rows past it - the
+// sum of squares over or the products h w over or under the range, a factor rstd / s over it
+// - are computed in the order of the formulas and from memory (`rare_row`).
+//
+// A row whose h, or whose y, are not all finite in FP32 gets a NaN scale; other rows are
 // unaffected.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -66,12 +70,21 @@ __device__ __forceinline__ float2 block_sum_max(float sum, float top) {
 }
 
 template <bool kE4M3>
+constexpr float kTop = kE4M3 ? 448.0f : 127.0f;
+
+// (scale, the codes' factor rstd / s) of a row.  The factor is 0, infinite or NaN where the
+// squares' mean, max|h w| or max|y| pass FP32 or the row is not finite, and where top /
+// max|h w| or rstd / 1e-30 do.  Elsewhere it is at most 2^128, so that a product h w that
+// falls among the subnormals (off by 2^-150) is off by 2^-22 of a code, and max|h w| either
+// above 2^-121, good to 2^-29 of itself, or without a part in the scale.
+template <bool kE4M3>
 __device__ __forceinline__ float2 row_scale(float2 stat, int width, float eps) {
   const float rstd = rsqrtf(stat.x / float(width) + eps);
-  float s = stat.y * rstd / (kE4M3 ? 448.0f : 127.0f);
+  float s = stat.y * rstd / kTop<kE4M3>;
   if (s < 1.0e-30f) s = 1.0e-30f;
   return make_float2(s, rstd / s);
 }
+__device__ __forceinline__ bool ordinary(float2 sc) { return sc.y > 0.0f && sc.y < INFINITY; }
 
 template <bool kE4M3>
 __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
@@ -84,6 +97,38 @@ __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
     asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, 0;" : "=r"(hi) : "r"(__float2int_rn(d)), "r"(__float2int_rn(c)));
     asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(w) : "r"(__float2int_rn(b)), "r"(__float2int_rn(a)), "r"(hi));
     return w;
+  }
+}
+
+// A row whose numbers leave FP32's range somewhere (see `ordinary`), by the block, from the
+// stored h: rstd first, so that h rstd <= sqrt(width), then the weight, then y / s.  Squares
+// that overflow are taken 2^100 smaller: the largest, 2^57 at least then, stays far above
+// FP32's smallest, and those that vanish beside it count for nothing.
+template <typename T, typename W, bool kE4M3>
+__device__ __forceinline__ void rare_row(const T* h, const W* w, uint8_t* q, float* scale, int width, float eps) {
+  __syncthreads();                       // the block's h is stored, its first statistics are read
+  float down = 1.0f, mean_eps = INFINITY;
+  for (int turn = 0; turn < 2 && !(mean_eps < INFINITY); ++turn) {
+    if (turn) down = 0x1p-100f;
+    float sum = 0.0f;
+    for (int c = threadIdx.x; c < width; c += blockDim.x) {
+      const float f = to_float(h[c]) * down;
+      sum = fmaf(f, f, sum);
+    }
+    mean_eps = block_sum_max(sum, 0.0f).x / float(width) + eps * down * down;
+    __syncthreads();
+  }
+  const float rstd = rsqrtf(mean_eps);   // of h * down; NaN or 0 where h is not finite
+  float top = 0.0f;
+  for (int c = threadIdx.x; c < width; c += blockDim.x)
+    top = max_nan(top, fabsf(to_float(h[c]) * down * rstd * to_float(w[c])));
+  float s = block_sum_max(0.0f, top).y / kTop<kE4M3>;
+  if (s < 1.0e-30f) s = 1.0e-30f;
+  if (!(s < INFINITY)) s = NAN;
+  if (threadIdx.x == 0) *scale = s;
+  for (int c = threadIdx.x; c < width; c += blockDim.x) {
+    const float y = to_float(h[c]) * down * rstd * to_float(w[c]) / s;
+    q[c] = uint8_t(codes4<kE4M3>(y, 0.0f, 0.0f, 0.0f));
   }
 }
 
@@ -136,6 +181,10 @@ __global__ void __launch_bounds__(kMaxThreads) rms_rows(const Args a) {
     }
   }
   const float2 sc = row_scale<kE4M3>(block_sum_max(sum, top), a.width, a.eps);
+  if (!ordinary(sc)) {
+    const T* from = r ? static_cast<const T*>(a.h) + row * a.hs : reinterpret_cast<const T*>(x);
+    return rare_row<T, W, kE4M3>(from, w, static_cast<uint8_t*>(a.q) + row * a.width, a.scale + row, a.width, a.eps);
+  }
   if (threadIdx.x == 0) a.scale[row] = sc.x;
   uint2* q = reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.q) + row * a.width);
 #pragma unroll
@@ -169,8 +218,8 @@ __device__ __forceinline__ void load_part(const T* row, int c0, int width, bool 
 // In tensors of one odd width every operand's vectors then fit, the codes' too (a code is
 // half as wide, and a vector of codes 8 bytes); an operand whose vectors do not goes value by
 // value.  The weights always do, from the L1 cache; the products with them are kept.
-// 16384 rows of 1537, BF16 with a residual: 58 us, 106 with every operand value by value; the
-// same rows of 1536 in rms_rows 30.  Bound by the instructions of the odd ends and weights.
+// 16384 rows of 1537, BF16 with a residual: 61 us, 106 with every operand value by value; the
+// same rows of 1536 in rms_rows 29.  Bound by the instructions of the odd ends and weights.
 template <typename T, typename W, bool kE4M3, int kVec>
 __global__ void __launch_bounds__(kMaxThreads + 32) rms_rows_any(const Args a) {
   const int64_t row = blockIdx.x;
@@ -216,6 +265,7 @@ __global__ void __launch_bounds__(kMaxThreads + 32) rms_rows_any(const Args a) {
     }
   }
   const float2 sc = row_scale<kE4M3>(block_sum_max(sum, top), a.width, a.eps);
+  if (!ordinary(sc)) return rare_row<T, W, kE4M3>(r ? ho : x, w, q, a.scale + row, a.width, a.eps);
   if (threadIdx.x == 0) a.scale[row] = sc.x;
 #pragma unroll
   for (int i = 0; i < kVec; ++i) {
@@ -235,9 +285,10 @@ __global__ void __launch_bounds__(kMaxThreads + 32) rms_rows_any(const Args a) {
 
 // Two vectors a thread, so that a row's loads are in flight together and the reduction has
 // few warps; four where the block would pass kMaxThreads, one in rows of at most 32 vectors.
-// With 1 / 2 / 4, BF16 with a residual, us: 16384 rows of 1536 35.4 / 29.7 / 31.4, of 4096
-// 96.6 / 72.1 / 74.2, of 5376 - / 97.9 / 100.7, of 256 10.7 / 10.9 / 11.2; of 1537
-// (rms_rows_any) 64.4 / 58.3 / 76.3, of 257 22.3 / 17.1 / 33.3; one row of 14336 4.3 (4).
+// With 1 / 2 / 4, BF16 with a residual, us, before rare_row was there: 16384 rows of 1536 35.4 /
+// 29.7 / 31.4, of 4096 96.6 / 72.1 / 74.2, of 5376 - / 97.9 / 100.7, of 256 10.7 / 10.9 / 11.2;
+// of 1537 (rms_rows_any) 64.4 / 58.3 / 76.3, of 257 22.3 / 17.1 / 33.3; one row of 14336 4.3 (4).
+// With it, as chosen: 29.3, 72.1, 96.4, 10.4; 60.8, 17.3.
 template <typename T, typename W, bool kE4M3>
 void launch(const Args& a, unsigned rows, bool vector, cudaStream_t stream) {
   const int vecs = vector ? a.width >> 3 : (a.width + 14) >> 3;   // with a first one that sticks out by 7

@@ -165,3 +165,68 @@ def test_feeds_the_int8_linear(device):
     want = (q.double() @ wq.double().T) * s.double() * ws.double()   # the integer sum is exact
     # one BF16 rounding of an FP32 value that was itself rounded three times
     assert torch.all((out.double() - want).abs() <= want.abs() * (2.0 ** -8 * 1.001))
+
+
+def definition_at(h, weight, dtype, eps):
+    h, w = h.double(), weight.double()
+    y = h / torch.sqrt(h.pow(2).mean(1, keepdim=True) + eps) * w
+    scale = (y.abs().amax(1, keepdim=True) / TOP[dtype]).clamp_min(1e-30)
+    return y / scale, scale
+
+
+FAR = [  # size of the values, of the FP32 weights, eps
+    (1e25, 1.0, 1e-6), (3e38, 1.0, 1e-6), (1e25, 1.0, 3e38), (2e19, 1e-20, 1e-6), (1e18, 1e21, 1e-6), (1e30, 1e30, 1e-6),
+    (1e-37, 1.0, 1e-20), (1e-37, 1.0, 1.2e-38), (3e-39, 1.0, 1.2e-38), (1e-10, 1e-30, 1e-30), (1e-25, 1e-15, 1.2e-38),
+    (1e-37, 1e30, 1e-20), (1e-20, 1.0, 1e-6), (1e4, 1e-35, 1e-6)]
+
+
+@pytest.mark.parametrize("size,by,eps", FAR)
+@pytest.mark.parametrize("dtype", list(TOP))
+@pytest.mark.parametrize("k", [1, 31, 256, 1155, 5376, 16381])
+def test_values_far_from_one(device, size, by, eps, dtype, k):
+    """Squares, products with the weights or the codes' factor that leave FP32's range, in
+    every BF16 row that the formulas give finite values for; beside ordinary rows, whose
+    bits do not change."""
+    x, _, w = make(5, k, torch.bfloat16, device, seed=3)
+    w, x = w.float() * by, x.float().clamp(-1, 1)
+    x = x / x.abs().amax(1, keepdim=True)
+    far = (x * size).to(torch.bfloat16)
+    q, s, _ = residual_rms_quant(far, w, eps=eps, dtype=dtype)
+    exact, want = definition_at(far, w, dtype, eps)
+    assert torch.all((s.double() - want).abs() <= 2e-6 * want)
+    # as in `check`: half a step of the codes, and the scale's part of a code
+    half = 0.5 if dtype == torch.int8 else torch.maximum(exact.abs() * 2.0 ** -4 * 1.0001, torch.tensor(2.0 ** -10))
+    assert torch.all((q.double() - exact).abs() <= half + TOP[dtype] * 4e-6)
+    mixed = torch.cat((make(3, k, torch.bfloat16, device)[0], far))
+    got = residual_rms_quant(mixed, w, eps=eps, dtype=dtype)
+    alone = residual_rms_quant(mixed[:3].contiguous(), w, eps=eps, dtype=dtype)
+    assert torch.equal(got[0][:3].view(torch.uint8), alone[0].view(torch.uint8)) and torch.equal(got[1][:3], alone[1])
+    assert torch.equal(got[0][3:].view(torch.uint8), q.view(torch.uint8)) and torch.equal(got[1][3:], s)
+
+
+@pytest.mark.parametrize("dtype", list(TOP))
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("eps", [1.2e-38, 1e-20, 1e-6, 3e38])
+def test_zero_rows_at_any_epsilon(device, dtype, t, eps):
+    for k in (64, 643):
+        x = torch.zeros((4, k), device=device, dtype=t)
+        x[2] = 1
+        for w in (torch.ones(k, device=device), torch.ones(k, device=device, dtype=t), torch.zeros(k, device=device)):
+            q, s, _ = residual_rms_quant(x, w, eps=eps, dtype=dtype)
+            zero = slice(None) if not w.any() else torch.tensor([0, 1, 3], device=device)
+            assert torch.all(q[zero].view(torch.uint8) == 0) and torch.all(s[zero] == torch.tensor(1e-30, device=device))
+
+
+def test_large_rows_of_a_stream_in_place(device):
+    """h beyond 2^64 in the caller's residual; and a row whose y passes FP32 is not finite."""
+    for k in (640, 643):
+        x, r, w = make(3, k, torch.bfloat16, device)
+        x, r = (x.float() * 1e30).bfloat16(), (r.float() * 1e30).bfloat16()
+        want = (x.float() + r.float()).bfloat16()
+        q, s, h = residual_rms_quant(x, w, residual=r, residual_out=r)
+        assert h is r and torch.equal(h, want)
+        check(q, s, h, w, torch.int8)
+        w = w.float()
+        w[7] = 3e38
+        x[1, 7] = 1e32
+        assert torch.isnan(residual_rms_quant(x, w)[1][1])
