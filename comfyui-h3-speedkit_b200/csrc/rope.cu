@@ -24,6 +24,7 @@
 #include <climits>
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "host_util.h"
 #include "wide_types.cuh"
@@ -136,6 +137,13 @@ __device__ __forceinline__ void fill_rotations(float2* cs, const Args& a, const 
   }
 }
 
+// BF16 squares can pass FP32: such a head is taken 2^100 smaller, its largest value then
+// 2^-46 at least.  (FP16 squares stay below 2^40.)  rsqrt of the mean is 0 there, NaN or 0 in
+// heads that are not finite.
+constexpr float kDown = 0x1p-100f;
+template <typename T, bool kNorm>
+constexpr bool kSquaresPass = kNorm && std::is_same<T, __nv_bfloat16>::value;
+
 // A lane's 16 channels of one head row.
 template <typename T>
 struct Chunk {
@@ -185,82 +193,106 @@ __global__ void __launch_bounds__(kThreads) rope_rows(const Args a, const __grid
     const int rows = tokens_of(tile) * heads;
     if (next < tiles)
       fill_rotations<true>(cs_buffers + (buffer ^ 1) * a.tile * token_size, a, own, next * a.tile, tokens_of(next));
-    // whole warps iterate together: the row's sum is a shuffle
-    for (int base = 0; base < rows; base += kUnroll * kStep) {
-      Chunk<T> ch[kUnroll];
+    const auto load = [&](int row, Chunk<T>& ch) {
+      const bool on = row < rows && active;
+      ch.t = row / heads;
+      const int head = head0 + row - ch.t * heads;
+      ch.is_q = head < a.q_heads;
+      const int h = ch.is_q ? head : head - a.q_heads;
+      const int64_t token = token0 + ch.t;
+      ch.dst = nullptr;
+      ch.u0 = ch.u1 = make_uint4(0, 0, 0, 0);
+      if (on) {
+        const T* src = ch.is_q ? static_cast<const T*>(a.q) + token * a.q_token + h * a.q_head
+                               : static_cast<const T*>(a.k) + token * a.k_token + h * a.k_head;
+        ch.dst = ch.is_q ? static_cast<T*>(a.qo) + token * a.qo_token + h * a.qo_head
+                         : static_cast<T*>(a.ko) + token * a.ko_token + h * a.ko_head;
+        ch.u0 = *reinterpret_cast<const uint4*>(src + c0);
+        ch.u1 = *reinterpret_cast<const uint4*>(src + c1);
+      }
+    };
+    // false for a head whose squares pass FP32: it is not written.  `smaller` takes such heads.
+    const auto turn = [&](const Chunk<T>& ch, auto smaller) -> bool {
+      bool fine = true;
+      float x[8], y[8];
+      unpack8<T>(ch.u0, x);
+      unpack8<T>(ch.u1, y);
+      if constexpr (kNorm) {
+        float sum = 0.0f, eps = a.eps;
+        if constexpr (smaller) {
+          eps = eps * kDown * kDown;
 #pragma unroll
-      for (int i = 0; i < kUnroll; ++i) {
-        const int row = base + i * kStep + int(threadIdx.x) / kLanes;
-        const bool on = row < rows && active;
-        ch[i].t = row / heads;
-        const int head = head0 + row - ch[i].t * heads;
-        ch[i].is_q = head < a.q_heads;
-        const int h = ch[i].is_q ? head : head - a.q_heads;
-        const int64_t token = token0 + ch[i].t;
-        ch[i].dst = nullptr;
-        ch[i].u0 = ch[i].u1 = make_uint4(0, 0, 0, 0);
-        if (on) {
-          const T* src = ch[i].is_q ? static_cast<const T*>(a.q) + token * a.q_token + h * a.q_head
-                                    : static_cast<const T*>(a.k) + token * a.k_token + h * a.k_head;
-          ch[i].dst = ch[i].is_q ? static_cast<T*>(a.qo) + token * a.qo_token + h * a.qo_head
-                                 : static_cast<T*>(a.ko) + token * a.ko_token + h * a.ko_head;
-          ch[i].u0 = *reinterpret_cast<const uint4*>(src + c0);
-          ch[i].u1 = *reinterpret_cast<const uint4*>(src + c1);
+          for (int e = 0; e < 8; ++e) x[e] *= kDown, y[e] *= kDown;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], fmaf(y[e], y[e], sum));
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (ch.dst) {
+          const float r = rsqrtf(sum / float(a.dim) + eps);
+          if (kSquaresPass<T, kNorm> && !smaller) fine = r > 0.0f;
+          float w0[8], w1[8];
+          if constexpr (kHeld) {
+            unpack8<W>(ch.is_q ? held[0] : held[2], w0);
+            unpack8<W>(ch.is_q ? held[1] : held[3], w1);
+          } else {
+            const W* w = static_cast<const W*>(ch.is_q ? a.qw : a.kw);
+            load8<W>(w + c0, w0);
+            load8<W>(w + c1, w1);
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            x[e] = x[e] * r * w0[e];
+            y[e] = y[e] * r * w1[e];
+          }
         }
       }
+      if (ch.dst) {
+        const float2* r = cs + ch.t * token_size + lane;   // pair 8 lane + e at r[e * eighths]
+        if constexpr (kInterleaved) {
+          const int left = a.pairs - 8 * lane;   // the lane's pairs that turn
 #pragma unroll
-      for (int i = 0; i < kUnroll; ++i) {
-        float x[8], y[8];
-        unpack8<T>(ch[i].u0, x);
-        unpack8<T>(ch[i].u1, y);
-        if constexpr (kNorm) {
-          float sum = 0.0f;
+          for (int e = 0; e < 8; ++e) {
+            float* v = e < 4 ? x + 2 * e : y + 2 * e - 8;
+            const float2 p = e < left ? r[e * eighths] : make_float2(1.0f, 0.0f);
+            const float v0 = v[0], v1 = v[1];
+            v[0] = v0 * p.x - v1 * p.y;
+            v[1] = v0 * p.y + v1 * p.x;
+          }
+        } else if (rotates) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], fmaf(y[e], y[e], sum));
-#pragma unroll
-          for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-          if (ch[i].dst) {
-            const float r = rsqrtf(sum / float(a.dim) + a.eps);
-            float w0[8], w1[8];
-            if constexpr (kHeld) {
-              unpack8<W>(ch[i].is_q ? held[0] : held[2], w0);
-              unpack8<W>(ch[i].is_q ? held[1] : held[3], w1);
-            } else {
-              const W* w = static_cast<const W*>(ch[i].is_q ? a.qw : a.kw);
-              load8<W>(w + c0, w0);
-              load8<W>(w + c1, w1);
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              x[e] = x[e] * r * w0[e];
-              y[e] = y[e] * r * w1[e];
-            }
+          for (int e = 0; e < 8; ++e) {
+            const float2 p = r[e * eighths];
+            const float x0 = x[e], x1 = y[e];
+            x[e] = x0 * p.x - x1 * p.y;
+            y[e] = x0 * p.y + x1 * p.x;
           }
         }
-        if (ch[i].dst) {
-          const float2* r = cs + ch[i].t * token_size + lane;   // pair 8 lane + e at r[e * eighths]
-          if constexpr (kInterleaved) {
-            const int left = a.pairs - 8 * lane;   // the lane's pairs that turn
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              float* v = e < 4 ? x + 2 * e : y + 2 * e - 8;
-              const float2 p = e < left ? r[e * eighths] : make_float2(1.0f, 0.0f);
-              const float v0 = v[0], v1 = v[1];
-              v[0] = v0 * p.x - v1 * p.y;
-              v[1] = v0 * p.y + v1 * p.x;
-            }
-          } else if (rotates) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float2 p = r[e * eighths];
-              const float x0 = x[e], x1 = y[e];
-              x[e] = x0 * p.x - x1 * p.y;
-              y[e] = x0 * p.y + x1 * p.x;
-            }
-          }
-          *reinterpret_cast<uint4*>(ch[i].dst + c0) = pack8<T>(x);
-          *reinterpret_cast<uint4*>(ch[i].dst + c1) = pack8<T>(y);
+        if (fine) {
+          *reinterpret_cast<uint4*>(ch.dst + c0) = pack8<T>(x);
+          *reinterpret_cast<uint4*>(ch.dst + c1) = pack8<T>(y);
         }
+      }
+      return fine;
+    };
+    // whole warps iterate together: the row's sum is a shuffle
+    uint32_t past = 0;   // a bit for each of the thread's rows, 16 at most
+    for (int base = int(threadIdx.x) / kLanes; base - int(threadIdx.x) / kLanes < rows; base += kUnroll * kStep) {
+      Chunk<T> ch[kUnroll];
+#pragma unroll
+      for (int i = 0; i < kUnroll; ++i) load(base + i * kStep, ch[i]);
+#pragma unroll
+      for (int i = 0; i < kUnroll; ++i) past = 2 * past + !turn(ch[i], std::false_type());
+    }
+    // (a check of each pair of rows in the loop: 185 us where this takes 179)
+    if (kSquaresPass<T, kNorm> && __any_sync(0xffffffffu, past != 0)) {
+      const int turns = (rows + kUnroll * kStep - 1) / (kUnroll * kStep) * kUnroll;
+#pragma unroll 1
+      for (int i = 0; i < turns; ++i) {
+        Chunk<T> ch;
+        load(int(threadIdx.x) / kLanes + i * kStep, ch);
+        if (!(past >> (turns - 1 - i) & 1u)) ch.dst = nullptr;
+        turn(ch, std::true_type());
       }
     }
   }
@@ -284,7 +316,8 @@ __global__ void __launch_bounds__(kThreads) rope_rows_scalar(const Args a, const
     __syncthreads();
     fill_rotations<false>(cs, a, own, token0, n);
     __syncthreads();
-    for (int row = threadIdx.x >> 5; row < rows; row += kThreads / 32) {
+    // false for a head whose squares pass FP32: it is not written.  `smaller` takes such heads.
+    const auto turn = [&](int row, auto smaller) -> bool {
       const int t = row / heads, head = head0 + row - t * heads;
       const bool is_q = head < a.q_heads;
       const int h = is_q ? head : head - a.q_heads;
@@ -298,12 +331,14 @@ __global__ void __launch_bounds__(kThreads) rope_rows_scalar(const Args a, const
       if (w) {
         float sum = 0.0f;
         for (int c = lane; c < a.dim; c += 32) {
-          const float x = to_float(src[c]);
+          float x = to_float(src[c]);
+          if constexpr (smaller) x *= kDown;
           sum = fmaf(x, x, sum);
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        r = rsqrtf(sum / float(a.dim) + a.eps);
+        r = rsqrtf(sum / float(a.dim) + (smaller ? a.eps * kDown * kDown : a.eps));
+        if (kSquaresPass<T, true> && !smaller && !(r > 0.0f)) return false;
       }
       // the pairs, then pairs of the channels that pass (a lane reads what it writes)
 #pragma unroll 2
@@ -312,6 +347,7 @@ __global__ void __launch_bounds__(kThreads) rope_rows_scalar(const Args a, const
         const int i0 = interleaved || !turns ? 2 * p : p, i1 = interleaved || !turns ? i0 + 1 : a.pairs + p;
         float x0 = to_float(src[i0]), x1 = to_float(src[i1]);
         if (w) {
+          if constexpr (smaller) x0 *= kDown, x1 *= kDown;
           x0 = x0 * r * to_float(w[i0]);
           x1 = x1 * r * to_float(w[i1]);
         }
@@ -324,6 +360,16 @@ __global__ void __launch_bounds__(kThreads) rope_rows_scalar(const Args a, const
         dst[i0] = from_float<T>(x0);
         dst[i1] = from_float<T>(x1);
       }
+      return true;
+    };
+    uint32_t past = 0;   // a bit for each of the warp's rows, 16 at most
+    const int first = threadIdx.x >> 5, step = kThreads / 32;
+    for (int row = first; row < rows; row += step) past = 2 * past + !turn(row, std::false_type());
+    if (kSquaresPass<T, true> && past) {
+      int row = first + (rows - 1 - first) / step * step;   // the warp's last, the lowest bit
+#pragma unroll 1
+      for (; past; past >>= 1, row -= step)
+        if (past & 1u) turn(row, std::true_type());
     }
   }
 }

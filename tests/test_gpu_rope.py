@@ -164,3 +164,26 @@ def test_stream_and_graph(device):
     again = rope_axes(q, k, at.flip(0).contiguous(), sections=(16, 16, 16))
     assert all(torch.equal(a, b) for a, b in zip(held, again))
     assert torch.equal(table, rope_table(held_at, sections=(16, 16, 16)))
+
+
+@pytest.mark.parametrize("size", [1e-30, 1e18, 1e19, 1e25, 3e38])
+@pytest.mark.parametrize("dim,sections,interleaved", [(128, (16, 16, 16), False), (64, (7, 9, 11), True), (256, (128,), False),
+                                                      (34, (3, 3), False), (128, (5,), False)])
+def test_norm_of_heads_of_any_size(device, size, dim, sections, interleaved):
+    """Squares past FP32 beside ordinary heads, whose bits do not change."""
+    q, k, at, _ = make(37, 5, 2, dim, torch.bfloat16, device, len(sections))
+    qw, kw = (1 + 0.2 * torch.randn(2, dim, device=device)).bfloat16()
+    go = lambda q: rope_axes(q, k, at, sections=sections, interleaved=interleaved, q_weight=qw, k_weight=kw)
+    plain = go(q)
+    far = q.float() / q.float().abs().amax(-1, keepdim=True) * size
+    mixed = q.clone()
+    mixed[:, ::2] = far[:, ::2].bfloat16()
+    got = go(mixed)
+    want = definition(mixed, at, sections, 10000.0, interleaved, qw)
+    close(got[0], want, want.abs().amax(-1, keepdim=True) * 2)
+    assert torch.equal(got[0][:, 1::2], plain[0][:, 1::2]) and torch.equal(got[1], plain[1])
+    mixed[3, 1, 2], mixed[4, 0, 1] = float("nan"), float("inf")
+    bad = go(mixed)[0]
+    assert torch.isnan(bad[3, 1]).all() and torch.isnan(bad[4, 0]).any()
+    bad[3, 1], bad[4, 0] = got[0][3, 1], got[0][4, 0]
+    assert torch.equal(bad, got[0])
