@@ -299,7 +299,7 @@ struct Softmax {
     }
   };
   // Scores in base 2 of 32 keys from key0 on, from the raw products.  cap tanh(y) comes
-  // without the exp2 unit where the warp's |y| are at most 1 (`small`); elsewhere as
+  // without the exp2 unit where |y| are at most 1 (`small`); elsewhere as
   // cap - 2 cap / (1 + e^(2y)), whose absolute error is a few 2^-24 of the cap too.
   static __device__ __forceinline__ void transform(uint32_t (&u)[32], const Args& a, const Cap& cap, bool small, float slope,
                                                    int pos, int key0) {
@@ -324,23 +324,35 @@ struct Softmax {
       for (int c = 0; c < 32; ++c) u[c] = __float_as_uint(fmaf(-slope, fabsf(d0 - float(c)), __uint_as_float(u[c])));
     }
   }
-  // whether every product of the warp's rows stays within |y| <= 1 (NaN does not)
-  static __device__ __forceinline__ bool all_small(const uint32_t (&x0)[32], const uint32_t (&x1)[32], const Args& a) {
+  // Whether the row's products stay within |y| <= 1 (NaN does not).  The choice moves last
+  // bits, and masked places hold anything.  So in a block that some row does not see whole
+  // each row chooses for itself, by what it sees; elsewhere the warp's rows, which see the
+  // same keys, choose together, but for those of no sequence (`idle`: a bit each).
+  template <bool kPart>
+  static __device__ __forceinline__ bool is_small(const uint32_t (&x0)[32], const uint32_t (&x1)[32], const Args& a,
+                                                   uint32_t idle, int from, int to) {
+    const uint32_t seen0 = seen(from, to), seen1 = seen(from - 32, to - 32);
+    const auto at = [](uint32_t x, uint32_t seen, int c) { return !kPart || (seen >> c) & 1u ? fabsf(__uint_as_float(x)) : 0.0f; };
     float m[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int c = 0; c < 32; c += 2) {
-      m[(c >> 1) & 1] = max3_nan(m[(c >> 1) & 1], fabsf(__uint_as_float(x0[c])), fabsf(__uint_as_float(x0[c + 1])));
-      m[2 + ((c >> 1) & 1)] = max3_nan(m[2 + ((c >> 1) & 1)], fabsf(__uint_as_float(x1[c])), fabsf(__uint_as_float(x1[c + 1])));
+      m[(c >> 1) & 1] = max3_nan(m[(c >> 1) & 1], at(x0[c], seen0, c), at(x0[c + 1], seen0, c + 1));
+      m[2 + ((c >> 1) & 1)] = max3_nan(m[2 + ((c >> 1) & 1)], at(x1[c], seen1, c), at(x1[c + 1], seen1, c + 1));
     }
-    return __all_sync(0xffffffffu, max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3])) * a.cap_y <= 1.0f);
+    const bool fits = max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3])) * a.cap_y <= 1.0f;
+    return kPart ? fits : (__ballot_sync(0xffffffffu, fits) | idle) == 0xffffffffu;
+  }
+  // bits of the places [from, to) of 32 keys
+  static __device__ __forceinline__ uint32_t seen(int from, int to) {
+    const int f = min(max(from, 0), 32), e = min(max(to, 0), 32);
+    const uint32_t below = e == 32 ? 0xffffffffu : (1u << e) - 1u, skip = f == 32 ? 0xffffffffu : (1u << f) - 1u;
+    return below & ~skip;
   }
   // -inf in the places outside [from, to) of 32 keys
   static __device__ __forceinline__ void mask(uint32_t (&u)[32], int from, int to) {
-    const int f = min(max(from, 0), 32), e = min(max(to, 0), 32);
-    const uint32_t below = e == 32 ? 0xffffffffu : (1u << e) - 1u, skip = f == 32 ? 0xffffffffu : (1u << f) - 1u;
-    const uint32_t seen = below & ~skip;
+    const uint32_t in = seen(from, to);
 #pragma unroll
-    for (int c = 0; c < 32; ++c) u[c] = (seen >> c) & 1u ? u[c] : 0xff800000u;
+    for (int c = 0; c < 32; ++c) u[c] = (in >> c) & 1u ? u[c] : 0xff800000u;
   }
   // what is taken off the scores before the exponential, twice
   static __device__ __forceinline__ uint64_t reference(float m) {
@@ -758,6 +770,7 @@ __global__ void __launch_bounds__(Form<kPair>::kThreads, Form<kPair>::kCtas)
     const uint64_t scale2 = pkf(scale, scale);
     const typename Soft::Cap cap(a);
     const float slope = (kFeat & kDistance) && valid ? a.slopes[head] * kLog2e : 0.0f;
+    const uint32_t idle = (kFeat & kCap) ? __ballot_sync(0xffffffffu, !valid) : 0u;   // the warp's rows of no sequence
     float m = -INFINITY, l = 0.0f;   // the reference maximum (base 2) and the sum
     bool ok = true;
     for (int n = 0; n < steps; ++n) {
@@ -775,7 +788,9 @@ __global__ void __launch_bounds__(Form<kPair>::kThreads, Form<kPair>::kCtas)
       const bool part = key0 < lo_max || key0 + kStep > hi_min;
       // a cap alone grows with the product, so the largest product gives the maximum and
       // the rest of the cap's polynomial goes into the probabilities
-      const bool small = (kFeat & kCap) && Soft::all_small(x0, x1, a), raw = kFeat == kCap && small && !part;
+      const bool small = (kFeat & kCap) && (part ? Soft::template is_small<true>(x0, x1, a, idle, lo - key0, hi - key0)
+                                                  : Soft::template is_small<false>(x0, x1, a, idle, 0, 0));
+      const bool raw = kFeat == kCap && small && !part;
       if ((kFeat || part) && !raw) {
         Soft::scores(x0, a, cap, small, slope, pos, key0, part, lo - key0, hi - key0);
         Soft::scores(x1, a, cap, small, slope, pos, key0 + 32, part, lo - key0 - 32, hi - key0 - 32);

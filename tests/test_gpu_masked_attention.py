@@ -469,3 +469,56 @@ def test_few_and_many_splits(device, rows, keys, d):
     assert plan(q, k)[2] > 1
     got = masked_attention(q, k, v, k_lengths=ints(lens, device), return_lse=True)
     check(got, definition(q, k, v, [(i, 0, rows, 0, n) for i, n in enumerate(lens)], scale=d ** -0.5))
+
+
+@pytest.mark.parametrize("distance", [False, True])
+@pytest.mark.parametrize("sq,sk,hq,hk", [(100, 200, 2, 2), (150, 333, 6, 2), (1, 3000, 14, 2), (1000, 1000, 74, 74)])
+def test_masked_places_move_no_bit(device, sq, sk, hq, hk, distance):
+    """Whatever keys and queries behind the sequences hold, under a cap: the same bits."""
+    q, k, v = make(1, sq, sk, hq, hk, 128, torch.bfloat16, device)
+    slopes = torch.exp2(-torch.arange(1, hq + 1, device=device).float() / hq) if distance else None
+    nq, nk = max(sq * 2 // 3, 1), sk * 3 // 4 + 1
+    for cap in (5.0, 40.0):
+        want = None
+        for fill in (0.0, 60.0, 3e38, NAN):
+            q[:, nq:], k[:, nk:], v[:, nk:] = fill, fill, fill
+            got = masked_attention(q, k, v, softcap=cap, slopes=slopes, q_lengths=ints([nq], device),
+                                   k_lengths=ints([nk], device), return_lse=True)
+            want = want or got
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("sq,sk,hq,hk", [(400, 400, 6, 2), (100, 64, 7, 1), (1000, 1000, 70, 10), (1, 3000, 24, 8)])
+def test_unused_rows_of_a_tile_move_no_bit(device, sq, sk, hq, hk):
+    """Rows that no query fills hold what an earlier kernel left in shared memory."""
+    q, k, v = make(1, sq, sk, hq, hk, 128, torch.bfloat16, device)
+    before = torch.zeros((1, 4096, 74, 128), device=device, dtype=torch.bfloat16)
+    want = None
+    for fill in (0.0, 30.0, NAN):
+        before[:] = fill
+        masked_attention(before, before[:, :64], before[:, :64])
+        got = masked_attention(q, k, v, softcap=30.0, return_lse=True)
+        want = want or got
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("distance", [False, True])
+@pytest.mark.parametrize("lens,heads", [([40, 70, 18, 300, 128], 2), ([900, 30, 1200, 7, 900], 40)])
+def test_other_documents_move_no_bit(device, lens, heads, distance):
+    """Documents that share tiles and key blocks, under a cap: what one of them holds does not
+    show in the others."""
+    offs = [sum(lens[:i]) for i in range(len(lens) + 1)]
+    q, k, v = make(1, offs[-1], offs[-1], heads, heads, 128, torch.bfloat16, device)
+    slopes = torch.exp2(-torch.arange(1, heads + 1, device=device).float() / heads) if distance else None
+    for cap in (5.0, 40.0):
+        clean = masked_attention(q, k, v, q_offsets=ints(offs, device), k_offsets=ints(offs, device), softcap=cap,
+                                 slopes=slopes, return_lse=True)
+        for fill in (60.0, 3e38, NAN):
+            a, b, c = q.clone(), k.clone(), v.clone()
+            for t in (a, b, c):
+                t[:, offs[1]:offs[2]], t[:, offs[3]:offs[4]] = fill, -fill
+            got = masked_attention(a, b, c, q_offsets=ints(offs, device), k_offsets=ints(offs, device), softcap=cap,
+                                   slopes=slopes, return_lse=True)
+            for i in (0, 2, 4):
+                rows = slice(offs[i], offs[i + 1])
+                assert torch.equal(got[0][:, rows], clean[0][:, rows]) and torch.equal(got[1][..., rows], clean[1][..., rows])
