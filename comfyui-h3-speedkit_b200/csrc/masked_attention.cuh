@@ -129,7 +129,7 @@ struct Smem {
   uint64_t v_full[kVStages], v_ok[kVStages], v_empty[kVStages];
   uint64_t s_full[F::kStreams], s_empty[F::kStreams], p_full[F::kStreams][2], pv_done[F::kStreams], done;   // P: step & 1
   int4 seen[F::kSoftWarps];        // a softmax warp's lowest and highest ends: lo min, lo max, hi min, hi max
-  int bad;                         // a V value that is not finite was met in a partly seen block
+  int bad;                         // a V value that is not finite and that some row sees, in a partly seen block
   uint32_t tmem;
   int abort;
   // an output row of every softmax thread crosses over the operand tiles
@@ -264,6 +264,38 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, int* abort,
 // The same by a whole warp, with one verdict.
 __device__ __forceinline__ bool all_wait(uint64_t* bar, uint32_t parity, int* abort, int* status, int code) {
   return __all_sync(0xffffffffu, wait(bar, parity, abort, status, code));
+}
+
+// The upper bits of a word's halves that are not finite values of the type.
+template <typename T>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+  constexpr uint32_t exponent = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
+  constexpr uint32_t carry = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
+  return ((w & exponent) + carry) & 0x80008000u;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t not_finite(const uint4& w) {
+  return not_finite<T>(w.x) | not_finite<T>(w.y) | not_finite<T>(w.z) | not_finite<T>(w.w);
+}
+
+// Clears a stage's values that are not finite, by a warp, and notes whether some row may see
+// one: those behind the last that one does, padding most of all, hold anything.
+template <typename T, int D, bool kPair>
+__device__ __forceinline__ void clear_not_finite(Smem<D, kPair>& sm, int stage, int key0, int hi_max) {
+  constexpr int kBlock = Form<kPair>::kBlock;
+  uint4* tile_v = reinterpret_cast<uint4*>(sm.v[stage]);
+#pragma unroll 1
+  for (int c = threadIdx.x & 31; c < Smem<D, kPair>::kTile / 16; c += 32) {
+    uint4 w = tile_v[c];
+    if (!not_finite<T>(w)) continue;
+    uint32_t* u = &w.x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) u[e] &= ~((not_finite<T>(u[e]) >> 15) * 0xffffu);
+    tile_v[c] = w;
+    const int key = key0 + ((c >> 3) & (kBlock - 1));   // (boxes of 64 channels, 128 bytes a key)
+    if (key < hi_max) sm.bad = 1;
+  }
+  fence_async_shared();
 }
 
 // FP16 probabilities are scaled by 2^7, away from that type's subnormals.
@@ -476,8 +508,14 @@ __device__ __forceinline__ void epilogue(const Args& a, Smem<D, kPair>& sm, uint
     if (valid && bad) {
       // values that are not finite, cleared from partly seen blocks, where this row sees them
       const T* v = static_cast<const T*>(a.v) + int64_t(batch * a.v_bmul) * a.v_sb + int64_t(kv_head * a.v_hmul) * a.v_sh + c;
-      for (int key = max(lo, first_key); key < min(hi, first_key + blocks * F::kBlock); ++key) {
-        if (!partial((key - first_key) / F::kBlock)) continue;
+      const int end = min(hi, first_key + blocks * F::kBlock);
+#pragma unroll 1
+      for (int key = max(lo, first_key); key < end; ++key) {
+        const int j = (key - first_key) / F::kBlock;
+        if (!partial(j)) {   // on to the next block
+          key = first_key + (j + 1) * F::kBlock - 1;
+          continue;
+        }
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
           const float y = to_float(v[int64_t(key) * a.v_ss + e]);
@@ -730,33 +768,17 @@ __global__ void __launch_bounds__(Form<kPair>::kThreads, Form<kPair>::kCtas)
       __syncwarp();
     } else {
       // ---------------- V check ----------------
-      const uint32_t mask = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
-      const uint32_t carry = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
       bool ok = true;
       for (int j = 0; ok && j < blocks; ++j) {
         const int s = j % S::kVStages;
         ok = all_wait(&sm.v_full[s], uint32_t(j / S::kVStages) & 1u, &sm.abort, a.status, 89);
         if (!ok) break;
         if (partial(j)) {
-          uint4* tile_v = reinterpret_cast<uint4*>(sm.v[s]);
-          bool found = false;
+          const uint4* tile_v = reinterpret_cast<const uint4*>(sm.v[s]);
+          uint32_t hits = 0;
 #pragma unroll 4
-          for (int c = lane; c < S::kTile / 16; c += 32) {
-            const uint4 w = tile_v[c];
-            const uint32_t hit = (((w.x & mask) + carry) | ((w.y & mask) + carry) | ((w.z & mask) + carry) |
-                                  ((w.w & mask) + carry)) & 0x80008000u;
-            if (hit) {
-              uint32_t u[4] = {w.x, w.y, w.z, w.w};
-              for (int e = 0; e < 4; ++e) {
-                const uint32_t h = ((u[e] & mask) + carry) & 0x80008000u;
-                u[e] &= ~((h >> 15) * 0xffffu);
-              }
-              tile_v[c] = make_uint4(u[0], u[1], u[2], u[3]);
-              found = true;
-            }
-          }
-          if (found) sm.bad = 1;
-          fence_async_shared();
+          for (int c = lane; c < S::kTile / 16; c += 32) hits |= not_finite<T>(tile_v[c]);
+          if (__any_sync(0xffffffffu, hits != 0)) clear_not_finite<T, D, kPair>(sm, s, first_key + j * F::kBlock, hi_max);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.v_ok[s]);

@@ -522,3 +522,49 @@ def test_other_documents_move_no_bit(device, lens, heads, distance):
             for i in (0, 2, 4):
                 rows = slice(offs[i], offs[i + 1])
                 assert torch.equal(got[0][:, rows], clean[0][:, rows]) and torch.equal(got[1][..., rows], clean[1][..., rows])
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("sq,sk,n", [(2048, 2048, 2000), (1, 30000, 29950), (300, 16384, 16300)])
+def test_padding_costs_nothing_by_what_it_holds(device, sq, sk, n, causal):
+    """NaN behind the sequence takes no longer than zeros there (it took 14 times as long)."""
+    q, k, v = make(1, sq, sk, 8, 8, 128, torch.bfloat16, device)
+    lengths = ints([n], device)
+
+    def ms():
+        times = []
+        for _ in range(7):
+            begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            begin.record()
+            for _ in range(5):
+                masked_attention(q, k, v, k_lengths=lengths, causal=causal)
+            end.record()
+            torch.cuda.synchronize()
+            times.append(begin.elapsed_time(end))
+        return sorted(times)[3]
+    v[:, n:] = 0
+    clean, want = ms(), masked_attention(q, k, v, k_lengths=lengths, causal=causal)
+    v[:, n:] = NAN
+    assert ms() < 2 * clean
+    assert torch.equal(masked_attention(q, k, v, k_lengths=lengths, causal=causal), want)
+
+
+@pytest.mark.parametrize("form", ["rows", "pairs", "split"])
+@pytest.mark.parametrize("d,t", [(128, torch.bfloat16), (64, torch.float16)])
+def test_values_not_finite_at_both_ends(device, form, d, t):
+    """V not finite at the first and the last key that rows see, NaN behind: it reaches the
+    rows that see it, in its channel, and nothing else."""
+    sq, sk, heads = dict(rows=(200, 700, 2), pairs=(1000, 1000, 74), split=(3, 20000, 2))[form]
+    q, k, v = make(1, sq, sk, heads, heads, d, t, device)
+    n = sk - 70
+    lengths = ints([n], device)
+    for causal in (False, True):
+        v0 = v.clone()
+        clean = masked_attention(q, k, v0, k_lengths=lengths, causal=causal)
+        v0[0, 0, 0, 5], v0[0, n - 1, 1, 33], v0[0, n // 2, 0, 60], v0[0, n:] = INF, NAN, -INF, NAN
+        out = masked_attention(q, k, v0, k_lengths=lengths, causal=causal)
+        at = torch.arange(sq, device=device) + (n - sq if causal else sk)      # the last key a row sees
+        want = clean.clone()
+        want[0, at >= 0, 0, 5], want[0, at >= n - 1, 1, 33], want[0, at >= n // 2, 0, 60] = INF, NAN, -INF
+        assert torch.equal(torch.isnan(out), torch.isnan(want))
+        assert torch.equal(out.nan_to_num(5.0), want.nan_to_num(5.0))
