@@ -3,12 +3,12 @@
 // of Python checks and ctypes took 26 to 43 us on the host, more than the kernels of
 // short inputs).  The work itself is libh3sk_b200.so's C entry points.
 //
-// A broken contract raises ValueError before anything is allocated or launched; a
-// CUDA error code raises RuntimeError.  Every operand is recorded on the current
+// A broken contract raises ValueError before anything is allocated or launched (operands as
+// the other operators take them: plain tensors without a gradient); a CUDA error code raises
+// RuntimeError.  Every operand is recorded on the current
 // stream of its device, and the caller's own outputs count as modified.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
-#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -65,14 +65,28 @@ bool normal_positive(double x) {
   return std::isfinite(x) && std::isfinite(f) && f >= FLT_MIN;
 }
 
-// One device, strided data, no recorded gradient.  The device itself is checked
-// last, so that the other rules hold on a host without a GPU too.
+// Tensors whose memory is their value: torch.Tensor itself, not a subclass (a Parameter, a
+// wrapper), nothing that is negated or conjugated on reading, or zero without memory.
+void original(const Maybe& t) {
+  if (!t) return;
+  const py::object object = py::reinterpret_steal<py::object>(THPVariable_Wrap(*t));
+  need(reinterpret_cast<PyObject*>(Py_TYPE(object.ptr())) == THPVariableClass && !t->is_neg() && !t->is_conj() &&
+           !t->_is_zerotensor() && t->layout() == at::kStrided,
+       "All operands must be original plain Torch tensors");
+}
+template <typename... Operands>
+void originals(const Operands&... operands) {
+  (original(operands), ...);
+}
+
+// One device, nothing that carries a gradient: recorded, to be recorded, or a forward-mode
+// tangent.  The device itself is checked last, so that the other rules hold on a host
+// without a GPU too.
 void plain(const List& operands) {
   const auto device = operands[0].t->device();
   for (const Named& o : operands) {
-    if (o.t->layout() != at::kStrided) refuse(std::string(o.name) + " must be a strided tensor");
     if (o.t->device() != device) refuse("All operands must use one CUDA device");
-    if (o.t->requires_grad() && c10::GradMode::is_enabled())
+    if (o.t->requires_grad() || o.t->_fw_grad(0).defined())
       refuse("Inference only; detach only after validating model autograd policy");
   }
 }
@@ -137,6 +151,7 @@ bool rows_ok(const Tensor& t, int64_t m, int64_t k, at::ScalarType type) {
 
 py::tuple rms_quant(const Tensor& x, const Tensor& weight, const Maybe& residual, double eps, int code, const Maybe& residual_out,
                     const Maybe& out, const Maybe& out_scale) {
+  originals(x, weight, residual, residual_out, out, out_scale);
   const int type = type_of(x);
   need(x.dim() == 2 && type >= 0, "x requires BF16 or FP16 [M,K]");
   const int64_t m = x.size(0), k = x.size(1);
@@ -251,6 +266,7 @@ bool slices_apart(const Tensor& a, const Tensor& b) {
 
 py::tuple rope_axes(const Tensor& q, const Maybe& k, const Tensor& positions, const Axes& axes, bool interleaved, bool inverse,
                     const Maybe& q_weight, const Maybe& k_weight, double eps, const Maybe& q_out, const Maybe& k_out) {
+  originals(q, k, positions, q_weight, k_weight, q_out, k_out);
   check_positions(positions, axes);
   const int type = type_of(q);
   need(q.dim() == 3 && type >= 0, "q requires BF16 or FP16 [T,H,D]");
@@ -313,6 +329,7 @@ py::tuple rope_axes(const Tensor& q, const Maybe& k, const Tensor& positions, co
 }
 
 Tensor rope_table(const Tensor& positions, const Axes& axes, const Maybe& out) {
+  originals(positions, out);
   check_positions(positions, axes);
   const int64_t tokens = positions.size(0), pairs = axes.pairs();
   const std::vector<int64_t> shape = {1, tokens, 1, pairs, 2, 2};
@@ -363,6 +380,7 @@ py::object masked_attention(const Tensor& q, const Tensor& k, const Tensor& v, s
                             const Maybe& slopes, bool causal, const Maybe& prefix, const Maybe& q_offsets, const Maybe& k_offsets,
                             const Maybe& q_lengths, const Maybe& k_lengths, const Maybe& out_arg, const Maybe& lse_arg,
                             bool return_lse) {
+  originals(q, k, v, slopes, prefix, q_offsets, k_offsets, q_lengths, k_lengths, out_arg, lse_arg);
   const int type = type_of(q);
   const bool flat = q.dim() == 3;
   for (const Tensor* t : {&q, &k, &v})

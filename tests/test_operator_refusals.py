@@ -271,3 +271,48 @@ def test_masked_attention_struct_and_nothing_to_do():
     assert lib.h3_masked_attention_run(None, 0) == INVALID and lib.h3_masked_attention_workspace(None) == -1
     assert lib.h3_masked_attention_plan(None, (ct.c_int * 3)()) == INVALID
     assert attention_args(batch=0, q=None) == 0 and attention_args(q_len=0, out=None) == 0
+
+
+class Subclass(torch.Tensor):
+    pass
+
+
+def kinds(t):
+    """A tensor as no operator of this package takes it: a subclass, a Parameter, one that is
+    negated on reading, one without memory."""
+    yield t.as_subclass(Subclass), "original plain"
+    yield torch.nn.Parameter(t, requires_grad=False), "original plain"
+    yield torch._neg_view(t), "original plain"
+    yield torch._efficientzerotensor(t.shape, dtype=t.dtype), "original plain"
+    yield t.clone().requires_grad_(), "Inference only"
+
+
+CALLS = {  # operator, operands by name
+    "rms_quant": (rms_quant.residual_rms_quant, lambda: dict(
+        x=x(), weight=torch.ones(32, dtype=BF), residual=x(), residual_out=x())),
+    "rope_axes": (rope.rope_axes, lambda: dict(
+        q=heads(), k=heads(), positions=at(dtype=torch.float32), sections=(8, 8, 8), q_weight=torch.ones(64),
+        k_weight=torch.ones(64), q_out=heads(), k_out=heads())),
+    "rope_table": (rope.rope_table, lambda: dict(
+        positions=at(dtype=torch.float32), sections=(8, 8, 8), out=torch.zeros((1, 4, 1, 24, 2, 2), dtype=BF))),
+    "masked_attention": (ma.masked_attention, lambda: qkv() | dict(
+        slopes=torch.zeros(4), out=torch.zeros((2, 5, 4, 64), dtype=BF), lse=torch.zeros((2, 4, 5)))),
+}
+
+
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("name", list(CALLS))
+def test_operands_are_plain_tensors_without_a_gradient(name, grad):
+    """Whether gradients are recorded at the time or not, as in the package's other operators."""
+    import torch.autograd.forward_ad as forward
+    call, operands = CALLS[name]
+    for key, t in operands().items():
+        if not isinstance(t, torch.Tensor):
+            continue
+        for other, text in kinds(t):
+            with torch.set_grad_enabled(grad), pytest.raises(ValueError, match=text):
+                call(**operands() | {key: other})
+        with forward.dual_level(), pytest.raises(ValueError, match="Inference only"):
+            call(**operands() | {key: forward.make_dual(t, torch.ones_like(t))})
+    with pytest.raises(ValueError, match="CUDA device"):     # and nothing else is wrong
+        call(**operands())
