@@ -356,12 +356,13 @@ Tensor rope_table(const Tensor& positions, const Axes& axes, const Maybe& out) {
 
 constexpr int64_t kMaxLength = int64_t(1) << 30;
 
-struct View {   // [B, S, H, D] of a 3-D or 4-D tensor; strides 0 for dimensions of one element
+struct View {   // [B, S, H, D] of a 3-D or 4-D tensor; strides 0 for dimensions of one element,
+                // and where there is none at all
   int64_t size[4], stride[3];
   explicit View(const Tensor& t) {
     const int64_t d = t.dim() - 4;   // -1: one sequence
     for (int i = 0; i < 4; ++i) size[i] = i + d < 0 ? 1 : t.size(i + d);
-    for (int i = 0; i < 3; ++i) stride[i] = i + d < 0 || size[i] <= 1 ? 0 : t.stride(i + d);
+    for (int i = 0; i < 3; ++i) stride[i] = i + d < 0 || size[i] <= 1 || t.numel() == 0 ? 0 : t.stride(i + d);
   }
 };
 

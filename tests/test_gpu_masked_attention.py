@@ -568,3 +568,12 @@ def test_values_not_finite_at_both_ends(device, form, d, t):
         want[0, at >= 0, 0, 5], want[0, at >= n - 1, 1, 33], want[0, at >= n // 2, 0, 60] = INF, NAN, -INF
         assert torch.equal(torch.isnan(out), torch.isnan(want))
         assert torch.equal(out.nan_to_num(5.0), want.nan_to_num(5.0))
+
+
+def test_no_keys_of_any_layout(device):
+    """An empty cache's strides and address are no one's business."""
+    q = torch.randn((2, 5, 4, 128), device=device).bfloat16()
+    buf = torch.empty((2, 9, 2, 133), device=device, dtype=torch.bfloat16)
+    for none in (buf[:, :0, :, 1:129], buf[:, 9:, :, 3:131], torch.empty((2, 2, 0, 128), device=device, dtype=q.dtype).transpose(1, 2)):
+        out, lse = masked_attention(q, none, none, return_lse=True)
+        assert torch.all(out == 0) and torch.all(lse == -INF)
