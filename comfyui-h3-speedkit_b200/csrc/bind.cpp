@@ -496,6 +496,9 @@ py::object masked_attention(const Tensor& q, const Tensor& k, const Tensor& v, s
 }  // namespace
 
 PYBIND11_MODULE(h3sk_torch, m) {
+  // the argument blocks go to the library by address
+  if (h3_rope_args_size() != sizeof(H3RopeArgs) || h3_masked_attention_args_size() != sizeof(H3MaskedAttentionArgs))
+    throw std::runtime_error("H3 SpeedKit B200 library and binding were built from different argument blocks; build both again");
   py::class_<Axes>(m, "Axes").def(py::init<const std::vector<int64_t>&, const std::vector<double>&>());
   m.def("rms_quant", &rms_quant);
   m.def("rope_axes", &rope_axes);

@@ -13,7 +13,8 @@ compiled without it and spells every epilogue rounding explicitly.  The QKV head
 epilogue is compiled without it and the K anchor detector and the INT8
 attention with it, as the reference compiles its qkv/sample, anchor and dense
 units (tools/build_kernels.py:30-37).  ``h3sk_torch.so`` beside the library is the
-PyTorch binding of the operators that are called once per token (``bind.cpp``).
+PyTorch binding of the operators that are called once per token (``bind.cpp``); the
+manifest's ``binding`` names the library, the torch and the Python it was made for.
 """
 from __future__ import annotations
 
@@ -21,11 +22,13 @@ import argparse
 import hashlib
 import json
 import os
+import platform
 import shutil
 import subprocess
 import sys
 import sysconfig
 from concurrent.futures import ThreadPoolExecutor
+from importlib import metadata
 from pathlib import Path
 
 CSRC = Path(__file__).resolve().parent
@@ -63,35 +66,41 @@ def nvcc_path(explicit: str | None = None) -> str:
     raise RuntimeError("nvcc not found; the CUDA toolkit is required to build the sm_100a library")
 
 
+def run(cmd: list[str]) -> subprocess.CompletedProcess:
+    return subprocess.run(cmd, text=True, capture_output=True)
+
+
+def hosts() -> dict:
+    """What the binding is compiled against; another of either needs another binding."""
+    return {"torch": metadata.version("torch"), "python": platform.python_version()}
+
+
 def up_to_date() -> bool:
-    lib = NATIVE / LIB_NAME
-    if not lib.exists() or not (NATIVE / BINDING_NAME).exists() or not (NATIVE / "build.json").exists():
+    built = (NATIVE / LIB_NAME, NATIVE / BINDING_NAME)
+    if not all(p.exists() for p in built) or not (NATIVE / "build.json").exists():
         return False
     newest = max(p.stat().st_mtime for p in [q for kind in ("*.cu", "*.cuh", "*.h", "*.cpp") for q in CSRC.glob(kind)]
                  + [PKG.parent / "include" / "h3sk_b200.h", Path(__file__)])
-    return lib.stat().st_mtime >= newest
+    if min(p.stat().st_mtime for p in built) < newest:
+        return False
+    binding = json.loads((NATIVE / "build.json").read_text()).get("binding", {})
+    return all(binding.get(name) == version for name, version in hosts().items())
 
 
-def build_binding() -> str:
-    """Compile bind.cpp against this interpreter's torch; returns the log."""
+def binding_command(library: Path, out: Path) -> list[str]:
+    """The command that compiles bind.cpp against this interpreter's torch and `library`."""
     import torch
     root = Path(torch.__file__).resolve().parent
     cuda = Path(nvcc_path()).resolve().parents[1]
     includes = [root / "include", root / "include/torch/csrc/api/include", sysconfig.get_paths()["include"], cuda / "include"]
-    tmp = NATIVE / (BINDING_NAME + ".tmp")
-    cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-DNDEBUG", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{p}" for p in includes),
-           str(CSRC / "bind.cpp"), "-o", str(tmp), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu",
-           "-ltorch_cuda", "-lc10", "-lc10_cuda", f"-L{NATIVE}", f"-l:{LIB_NAME}", "-Wl,-rpath,$ORIGIN"]
-    result = subprocess.run(cmd, text=True, capture_output=True)
-    log = f"$ {' '.join(cmd)}\n{result.stdout}{result.stderr}"
-    if result.returncode:
-        raise RuntimeError(f"g++ failed on bind.cpp:\n{result.stderr[-6000:]}")
-    os.replace(tmp, NATIVE / BINDING_NAME)
-    return log
+    return ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-DNDEBUG", "-fvisibility=hidden",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{p}" for p in includes),
+            str(CSRC / "bind.cpp"), "-o", str(out), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu",
+            "-ltorch_cuda", "-lc10", "-lc10_cuda", f"-L{library.parent}", f"-l:{library.name}", "-Wl,-rpath,$ORIGIN"]
 
 
 def build(nvcc: str | None = None, force: bool = False, quiet: bool = True) -> Path:
+    """Build the library and the binding, and put both in place only when both are there."""
     if not force and up_to_date():
         return NATIVE / LIB_NAME
     nvcc = nvcc_path(nvcc)
@@ -100,29 +109,35 @@ def build(nvcc: str | None = None, force: bool = False, quiet: bool = True) -> P
     version = subprocess.check_output([nvcc, "--version"], text=True)
     manifest = {"schema": 1, "status": "building", "target": "sm_100a", "nvcc": version, "kernels": {}}
     objects, logs, commands = [], [], {}
+
+    def done(what, cmd, result):
+        logs.append(f"$ {' '.join(cmd)}\n{result.stdout}{result.stderr}")
+        if result.returncode:
+            (NATIVE / "build.log").write_text("\n".join(logs))
+            raise RuntimeError(f"{what}:\n{result.stderr[-6000:]}")
+
     for source, extra in UNITS:
         src = CSRC / source
         commands[source] = [nvcc, *COMMON, *ARCH, *extra, "-c", str(src), "-o", str(BUILD / (src.stem + ".o"))]
         objects.append(BUILD / (src.stem + ".o"))
     with ThreadPoolExecutor(os.cpu_count() or 1) as pool:
-        results = list(pool.map(lambda cmd: subprocess.run(cmd, text=True, capture_output=True), commands.values()))
+        results = list(pool.map(run, commands.values()))
     for (source, cmd), result in zip(commands.items(), results):
-        logs.append(f"$ {' '.join(cmd)}\n{result.stdout}{result.stderr}")
-        if result.returncode:
-            (NATIVE / "build.log").write_text("\n".join(logs))
-            raise RuntimeError(f"nvcc failed on {source}:\n{result.stderr[-6000:]}")
-    lib = NATIVE / LIB_NAME
-    tmp = NATIVE / (LIB_NAME + ".tmp")
-    link = [nvcc, *ARCH, "-shared", "-Xcompiler", "-fPIC", *map(str, objects), "-o", str(tmp)]
-    result = subprocess.run(link, text=True, capture_output=True)
-    logs.append(f"$ {' '.join(link)}\n{result.stdout}{result.stderr}")
-    (NATIVE / "build.log").write_text("\n".join(logs))
-    if result.returncode:
-        raise RuntimeError(f"link failed:\n{result.stderr[-4000:]}")
-    os.replace(tmp, lib)
-    logs.append(build_binding())
+        done(f"nvcc failed on {source}", cmd, result)
+    lib, binding = BUILD / LIB_NAME, BUILD / BINDING_NAME
+    link = [nvcc, *ARCH, "-shared", "-Xcompiler", "-fPIC", *map(str, objects), "-o", str(lib)]
+    done("link failed", link, run(link))
+    bind = binding_command(lib, binding)
+    done("g++ failed on bind.cpp", bind, run(bind))
+    # an interruption from here on leaves no manifest, so that the next build starts again
+    (NATIVE / "build.json").unlink(missing_ok=True)
+    os.replace(lib, NATIVE / LIB_NAME)
+    os.replace(binding, NATIVE / BINDING_NAME)
+    lib, binding = NATIVE / LIB_NAME, NATIVE / BINDING_NAME
     (NATIVE / "build.log").write_text("\n".join(logs))
     digest = sha256(lib)
+    manifest["binding"] = {"source": "csrc/bind.cpp", "source_sha256": sha256(CSRC / "bind.cpp"), "command": bind,
+                           "file": BINDING_NAME, "sha256": sha256(binding), "library_sha256": digest, **hosts()}
     sources = {"norm": "norm_quant.cu", "residual": "norm_quant.cu", "convrot": "convrot_quant.cu",
                "fc1": "int8_gemm.cu", "gate": "int8_gemm.cu", "qkv": "qkv_quant.cu", "sample": "qkv_quant.cu",
                "anchor": "anchor.cu", "dense": "attention.cu"}

@@ -1,5 +1,6 @@
 // Host side of the attention under masks: argument checks, the cut of the work, tensor maps
 // and launches of masked_attention.cuh's kernels, and the BF16 ones themselves.
+#include "../../include/h3sk_b200.h"
 #include "masked_attention.cuh"
 
 namespace h3sk {
@@ -32,22 +33,6 @@ bool encode(CUtensorMap* map, const void* base, bool bf16, int rank, const uint6
 }  // namespace h3sk
 
 #define H3SK_EXPORT extern "C" __attribute__((visibility("default")))
-
-struct H3MaskedAttentionArgs {
-  const void *q, *k, *v;
-  void* out;
-  float* lse;
-  const float* slopes;
-  const int *q_offsets, *k_offsets, *q_lengths, *k_lengths, *prefix;
-  void* workspace;
-  uint64_t workspace_bytes;
-  int64_t q_stride_b, q_stride_s, q_stride_h;
-  int64_t k_stride_b, k_stride_s, k_stride_h;
-  int64_t v_stride_b, v_stride_s, v_stride_h;
-  int64_t o_stride_b, o_stride_s, o_stride_h;
-  int32_t batch, q_len, k_len, q_heads, k_heads, dim, type, documents, causal, fill;
-  float scale, softcap;
-};
 
 namespace h3sk {
 namespace mattn {

@@ -26,6 +26,7 @@
 #include <cstdint>
 #include <type_traits>
 
+#include "../../include/h3sk_b200.h"
 #include "host_util.h"
 #include "wide_types.cuh"
 
@@ -443,21 +444,6 @@ bool fill_tables(Tables* tb, const double* turns, const int* axis, int pairs, in
 }  // namespace h3sk
 
 #define H3SK_EXPORT extern "C" __attribute__((visibility("default")))
-
-struct H3RopeArgs {
-  const void *q, *k;
-  void *q_out, *k_out;
-  const void *q_weight, *k_weight;
-  const void* positions;
-  const double* turns;   // host, [pairs]
-  const int* axis;       // host, [pairs]
-  int64_t tokens;
-  int64_t q_stride_t, q_stride_h, k_stride_t, k_stride_h;
-  int64_t qo_stride_t, qo_stride_h, ko_stride_t, ko_stride_h;
-  int32_t q_heads, k_heads, dim, pairs, axes;
-  int32_t float_positions, type, weight_type, interleaved, inverse;
-  float eps;
-};
 
 H3SK_EXPORT size_t h3_rope_args_size(void) { return sizeof(H3RopeArgs); }
 

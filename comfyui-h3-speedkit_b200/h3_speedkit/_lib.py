@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes as ct
 import importlib.machinery
 import importlib.util
+import json
 import threading
 from pathlib import Path
 
@@ -121,7 +122,7 @@ def binding():
     beside it: the operators whose whole call has to take microseconds."""
     global _binding
     if _binding is None:
-        import torch  # noqa: F401  (its libraries are the binding's)
+        import torch  # (its libraries are the binding's)
         load()
         with _lock:
             if _binding is None:
@@ -129,6 +130,10 @@ def binding():
                 if not target.exists():
                     raise RuntimeError(f"H3 SpeedKit B200 binding not found at {target}; build it with "
                                        "`python comfyui-h3-speedkit_b200/csrc/build.py` (no fallback exists)")
+                made = json.loads(manifest.read_text()).get("binding", {}) if (manifest := NATIVE / "build.json").exists() else {}
+                if made.get("torch", torch.__version__) != torch.__version__:
+                    raise RuntimeError(f"H3 SpeedKit B200 binding was built for torch {made['torch']}, this is "
+                                       f"{torch.__version__}; run `python comfyui-h3-speedkit_b200/csrc/build.py`")
                 loader = importlib.machinery.ExtensionFileLoader("h3sk_torch", str(target))
                 module = importlib.util.module_from_spec(importlib.util.spec_from_loader("h3sk_torch", loader))
                 loader.exec_module(module)
