@@ -18,6 +18,8 @@ rounded once.  ``MaskedAttentionProvider`` puts it, with the rotary positions, b
 """
 from __future__ import annotations
 
+import torch
+
 from .. import _lib
 from .rope import rope_axes
 
@@ -75,7 +77,10 @@ class MaskedAttentionProvider:
             raise ValueError('The projection does not divide into the heads')
         q, k, v = (t.view(m, self.heads, width // self.heads) for t in (q, k, v))
         if self.positions is not None:
-            w = [None if t is None else t.detach().to(device=q.device, dtype=q.dtype).contiguous() for t in (q_weight, k_weight)]
+            # both as they are stored, in FP32 if either is (or is of another type)
+            own = all(t is None or t.dtype == q.dtype for t in (q_weight, k_weight))
+            w = [None if t is None else t.detach().to(device=q.device, dtype=q.dtype if own else torch.float32).contiguous()
+                 for t in (q_weight, k_weight)]
             q, k = rope_axes(q, k, self.positions, q_weight=w[0], k_weight=w[1], eps=eps, **self.rope)
         elif q_weight is not None:
             raise ValueError('A block with per-head norms needs positions')

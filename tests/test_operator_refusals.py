@@ -1,6 +1,7 @@
 """What the norm-quantiser, the rotary positions and the masked attention refuse, before
 any CUDA call."""
 import ctypes as ct
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -316,3 +317,19 @@ def test_operands_are_plain_tensors_without_a_gradient(name, grad):
             call(**operands() | {key: forward.make_dual(t, torch.ones_like(t))})
     with pytest.raises(ValueError, match="CUDA device"):     # and nothing else is wrong
         call(**operands())
+
+
+@pytest.mark.parametrize("q_type,k_type,want", [(BF, BF, BF), (torch.float32, torch.float32, torch.float32),
+                                                (BF, torch.float32, torch.float32), (torch.float16, torch.float16, torch.float32)])
+def test_provider_keeps_the_norm_weights_digits(monkeypatch, q_type, k_type, want):
+    """Norm weights reach the rotation as they are stored: a BF16 Q does not round FP32 ones."""
+    weights = [(1 + 0.1 * torch.arange(128) / 128).to(t) for t in (q_type, k_type)]
+    block = SimpleNamespace(attn=SimpleNamespace(**{n: SimpleNamespace(weight=torch.nn.Parameter(w), eps=1e-6)
+                                                    for n, w in zip(("q_norm", "k_norm"), weights)}))
+    seen = {}
+    monkeypatch.setattr(ma, "rope_axes", lambda q, k, at, **more: seen.update(more) or (q, k))
+    monkeypatch.setattr(ma, "masked_attention", lambda q, k, v, **masks: v)
+    provider = ma.MaskedAttentionProvider(2, positions=at(), sections=(16, 16, 16))
+    provider.for_block(block)(*(torch.zeros((4, 256), dtype=BF) for _ in range(3)))
+    for name, w in zip(("q_weight", "k_weight"), weights):
+        assert seen[name].dtype == want and torch.equal(seen[name].double(), w.double())
