@@ -58,9 +58,13 @@ class MaskedAttentionProvider:
     block's ``attn.q_norm`` / ``attn.k_norm``; called directly, without a block, Q and
     K are not normalised."""
 
+    MASKS = ('scale', 'softcap', 'slopes', 'causal', 'prefix', 'q_offsets', 'k_offsets', 'q_lengths', 'k_lengths')
+
     def __init__(self, heads, *, positions=None, sections=None, theta=10000.0, interleaved=False, **masks):
         if (positions is None) != (sections is None):
             raise ValueError('positions and sections are given together')
+        if not set(masks) <= set(self.MASKS):
+            raise ValueError(f'masks are any of {", ".join(self.MASKS)}')
         self.heads, self.positions, self.masks = heads, positions, masks
         self.rope = dict(sections=sections, theta=theta, interleaved=interleaved)
 

@@ -333,3 +333,11 @@ def test_provider_keeps_the_norm_weights_digits(monkeypatch, q_type, k_type, wan
     provider.for_block(block)(*(torch.zeros((4, 256), dtype=BF) for _ in range(3)))
     for name, w in zip(("q_weight", "k_weight"), weights):
         assert seen[name].dtype == want and torch.equal(seen[name].double(), w.double())
+
+
+def test_provider_takes_masks_alone():
+    """The block wants the attention's result and nothing else: no outputs of the caller's, no lse."""
+    for other in (dict(return_lse=True), dict(out=torch.zeros((4, 2, 64), dtype=BF)), dict(lse=torch.zeros((2, 4))), dict(mask=None)):
+        with pytest.raises(ValueError, match="masks are any of"):
+            ma.MaskedAttentionProvider(2, causal=True, **other)
+    assert ma.MaskedAttentionProvider(2, causal=True, softcap=3.0).masks == dict(causal=True, softcap=3.0)
