@@ -276,7 +276,8 @@ class ModelPatch:
         self.lock = threading.RLock()
         self.last_report = {}
         self.warned = set()
-        self.verify_new_shapes = verify_new_shapes
+        # a provider of other attention than the block's own cannot repeat the block's bits
+        self.verify_new_shapes = verify_new_shapes and not isinstance(attention, MaskedAttentionProvider)
         self.verified_shapes = Counter()
         self.rejected_shapes = set()
 
@@ -362,7 +363,9 @@ def patch_model(model, directory=None, *, release_embeddings=True, verify_new_sh
     """Return a Comfy clone with explicit block replacements and a request
     wrapper (runtime.py:311-338).  The original model is not modified.
     attention: "int8" (the reference's QKV op and INT8 attention, the default) or
-    a callable provider on the BF16 Q/K/V slices (MaskedAttentionProvider); None (identity) is refused."""
+    a callable provider on the BF16 Q/K/V slices; None (identity) is refused.
+    A MaskedAttentionProvider runs without the exact verification of new shapes, which holds
+    the patched block to the original one's bits: its attention is another by intent."""
     import comfy.patcher_extension as pe
     if attention is None:
         raise Unsupported("The B200 path needs an attention provider: 'int8' or a callable (None is identity)")

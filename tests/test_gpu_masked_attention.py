@@ -577,3 +577,28 @@ def test_no_keys_of_any_layout(device):
     for none in (buf[:, :0, :, 1:129], buf[:, 9:, :, 3:131], torch.empty((2, 2, 0, 128), device=device, dtype=q.dtype).transpose(1, 2)):
         out, lse = masked_attention(q, none, none, return_lse=True)
         assert torch.all(out == 0) and torch.all(lse == -INF)
+
+
+def test_patched_model_runs_the_provider(device):
+    """A patched model's block gives the provider's result, by default too (verification against
+    the block's own attention would put the original's in its place), and reports no fallback."""
+    from h3_speedkit import synthetic
+    from h3_speedkit.runtime import Backend, ModelPatch
+    from test_gpu_attention import _h3_block_ns
+    m, d, heads = 300, 512, 4
+    bw = synthetic.cfg5_block(0, d, 1024, tables=2, device=device)
+    block = _h3_block_ns(bw, *(torch.rand((2, 128), device=device) + 0.5).bfloat16())
+    at = torch.arange(m, device=device, dtype=torch.int32)[:, None].repeat(1, 3)
+    provider = MaskedAttentionProvider(heads, positions=at, sections=(16, 16, 16), causal=True)
+    x, t_emb, segments = synthetic.cfg5_tokens(m, d, device=device), torch.zeros((1, 4), device=device), [(0, 100, 0), (100, m, 1)]
+    backend = Backend()
+    want = x.clone()
+    backend.block(block, want, t_emb, segments, rows=(torch.arange(m, device=device) >= 100).int(), attention=provider)
+    patch = ModelPatch(SimpleNamespace(blocks=[block]), backend, attention=provider, blocks=1)
+    original = lambda inputs: {"img": torch.zeros_like(inputs["img"])}
+    run = lambda x: patch.replacement(0)(dict(img=x, t_emb=t_emb, mod_segments=segments), dict(original_block=original))["img"]
+    with torch.no_grad():
+        for _ in range(2):
+            got = patch.wrapper(run, x.clone())
+            assert torch.equal(got, want)
+            assert "fallback" not in patch.last_report and patch.last_report["counts"]["attention"] == 1
