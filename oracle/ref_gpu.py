@@ -21,14 +21,20 @@ class NotBuilt(FileNotFoundError):
     """The reference's kernel library is not there to compare with."""
 
 
+MISSING: set[str] = set()   # libraries that were asked for and are not there
+
+
 def available(name: str) -> bool:
-    return (REF / name).exists()
+    if (REF / name).exists():
+        return True
+    MISSING.add(name)
+    return False
 
 
 def _load(name: str) -> ct.CDLL:
     if name not in _CACHE:
         path = REF / name
-        if not path.exists():
+        if not available(name):
             raise NotBuilt(f"reference GPU oracle {path} is not built (run oracle/build.py)")
         _CACHE[name] = ct.CDLL(str(path), mode=ct.RTLD_LOCAL)
     return _CACHE[name]
