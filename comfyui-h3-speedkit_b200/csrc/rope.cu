@@ -490,11 +490,22 @@ H3SK_EXPORT int h3_rope_axes_run(const H3RopeArgs* r, uintptr_t stream_ptr) {
   a.float_positions = r->float_positions;
   a.eps = r->eps;
   a.sign = r->inverse ? -1.0f : 1.0f;
-  // Four steps of the CTA's threads to a tile, so that few tokens still spread over the
-  // SMs; sixteen where there are many (16384 tokens, 56 + 56 heads: 205 us with four, 188
-  // with sixteen).  A token's heads share its sines.
-  const int step = lanes ? kThreads / lanes : kThreads / 32, want = (r->tokens < 4096 ? 4 : 16) * step, heads = r->q_heads + r->k_heads;
-  a.chunk = r->tokens < 128 ? (heads < step ? heads : step) : (heads < want ? heads : want);
+  // Rows (a token's head) that a CTA's threads take at once are a step; a tile is as many steps
+  // as leave every SM work: 1, 2, 4, 8 or 16, by the steps that an SM has in all.  Longer
+  // tiles share a token's sines and overlap more, shorter ones spread over the SMs.  Us with
+  // 1 / 2 / 4 / 8 / 16 (heads of 128, normalised; steps an SM):
+  //   64 tokens, 8 heads (0.1): 3.3 / 3.9 / 5.5 / 5.5 / 5.5;  1024, 8 (1.7): 3.9 / 4.2 / 5.8 / 5.7 / 5.6
+  //   2048, 8 (3.5): 5.6 / 4.7 / 5.8 / 5.9 / 5.8;  256, 112 (6.1): 8.3 / 7.2 / 6.1 / 7.4 / 11.8
+  //   1024, 112 (24): 21.9 / 15.6 / 14.9 / 15.3 / 14.9;  16384, 32 (111): 85.6 / 61.3 / 58.8 / 60.5 / 64.0
+  //   8192, 112 (194): 163 / 111 / 103 / 97.1 / 98.5;  16384, 112 (387): 321 / 218 / 203 / 189 / 180
+  // heads of 64: 2048, 112 (24): 20.8 / 15.1 / 14.4 / 14.8 / 16.3;  16384, 112 (194): 160 / 110 / 102 / 96.2 / 96.6
+  int device = 0, sms = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
+    return cudaErrorInvalidDevice;
+  const int step = lanes ? kThreads / lanes : kThreads / 32, heads = r->q_heads + r->k_heads;
+  const int64_t per_sm = r->tokens * heads / (int64_t(step) * sms);
+  const int want = step * (per_sm < 2 ? 1 : per_sm < 6 ? 2 : per_sm < 144 ? 4 : per_sm < 288 ? 8 : 16);
+  a.chunk = heads < want ? heads : want;
   a.tile = a.chunk == heads ? want / heads : 1;
   if (a.tile > kMaxTile) a.tile = kMaxTile;
   if (a.tile < 1) a.tile = 1;

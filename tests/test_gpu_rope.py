@@ -187,3 +187,18 @@ def test_norm_of_heads_of_any_size(device, size, dim, sections, interleaved):
     assert torch.isnan(bad[3, 1]).all() and torch.isnan(bad[4, 0]).any()
     bad[3, 1], bad[4, 0] = got[0][3, 1], got[0][4, 0]
     assert torch.equal(bad, got[0])
+
+
+@pytest.mark.parametrize("tokens,hq,hk", [(70, 6, 2), (1500, 6, 2), (2500, 6, 2), (300, 60, 52), (700, 130, 70), (9000, 60, 52),
+                                          (17000, 60, 52), (16500, 20, 12)])
+@pytest.mark.parametrize("dim,sections,norm", [(128, (16, 16, 16), True), (64, (7, 9, 11), False)])
+def test_a_call_is_its_tokens_calls(device, tokens, hq, hk, dim, sections, norm):
+    """However the rows are cut into tiles: the bits of calls on pieces of the tokens and heads."""
+    q, k, at, _ = make(tokens, hq, hk, dim, torch.bfloat16, device, len(sections))
+    w = (1 + 0.2 * torch.randn(dim, device=device)).bfloat16() if norm else None
+    whole = rope_axes(q, k, at, sections=sections, q_weight=w, k_weight=w)
+    for cut in (slice(0, 1), slice(tokens // 3, tokens // 3 + 65), slice(tokens - 40, None)):
+        part = rope_axes(q[cut], None, at[cut].contiguous(), sections=sections, q_weight=w)[0]
+        assert torch.equal(part, whole[0][cut])
+        part = rope_axes(q[cut, :1], k[cut, -1:], at[cut].contiguous(), sections=sections, q_weight=w, k_weight=w)
+        assert torch.equal(part[0], whole[0][cut, :1]) and torch.equal(part[1], whole[1][cut, -1:])
