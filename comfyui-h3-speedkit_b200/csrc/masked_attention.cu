@@ -48,19 +48,27 @@ struct Plan {
 // tiles a group instead of ceil(S / 128) a head: the fewer tiles win.
 //
 // A CTA takes a pair of tiles (K and V blocks shared) or one tile, two CTAs an SM.  128 keys
-// cost 2.0 us a pair, 2.1 a single tile beside another, 1.3 one that has its SM alone; a
-// CTA's beginning and end 6.  The form with the shorter estimate runs: the longest CTA, or
-// all of them shared out over the SMs, a last round counting half where pairs run and a
-// quarter where single tiles do.  Measured pairs / single tiles, us: causal 6000 x 6000, 8
-// over 2 heads 95 / 82; causal 2048 x 2048, 16 heads 40 / 34; 1500 x 1500, 56 heads 90 / 81;
-// 512 x 512, 24 heads 17 / 13; 8192 x 8192, 24 heads 718 / 727; 21 documents in 12288
-// tokens, 16 over 4 heads 155 / 167.
+// cost 2.0 us a pair, 2.06 a single tile beside another, 1.3 one that has its SM alone; a
+// CTA's beginning and end 8.5 and 6.  The form with the shorter estimate runs: the longest
+// CTA, or all of them shared out over the SMs, a last round counting half where pairs run and
+// a quarter where single tiles do.  Measured pairs / single tiles in turn, at 1.6 to 1.7 GHz,
+// us: 8192 x 8192, 24 heads 819 / 772; 4096 x 4096, 8 heads 67 / 64; 2048 x 2048, 74 heads 177 /
+// 163; causal 6000 x 6000, 8 over 2 heads 94 / 78; 16384 x 16384, 8 heads 1074 / 1007, 16
+// heads 1963 / 2000, 56 heads 6833 / 6977.  16 over 4 heads of 12288 tokens in 2 / 5 / 21 / 60 /
+// 200 equal documents 615 / 288 / 116 / 74 / 61 against 568 / 269 / 104 / 65 / 50; in 21 ragged
+// ones 165 / 151.  Under a cap 6000 x 6000, 8 over 2 heads 271 / 222; 4096 x 4096, 8 heads 95.6 /
+// 96.6.
+// CTAs of at most ten blocks are taken at 2.0 and 2.1 with 6 for either, which gives pairs
+// where they fill whole rounds.  (Single tiles measured 4 to 10 % shorter there too: 1000 x
+// 1000, 74 heads 44 / 42, causal 34 / 31; 256 x 20000, 8 heads in 18 splits 33.5 / 32.0.  Their
+// plans stay as they were.)
 //
-// When the CTAs do not fill the SMs the keys are split beyond 512: at least 256 to a CTA,
-// 128 where there is one tile of rows and the splits are at most 16.  At least 128 / 256 /
-// 512 / 1024, us: 1 query x 1000 keys, 12 over 3 heads 11.0 / 11.9 / 14.3 / 16.5; x 2048,
-// batch 2, 24 over 4 10.7 / 11.8 / 13.7 / 18.9; x 8192, 28 over 4 13.5 / 12.1 / 14.2 / 19.7;
-// 1000 x 1000, 6 heads 19.5 / 17.7 / 18.2 / 18.2; 1 query x 300 keys 9.9 / 9.5 unsplit.
+// When the CTAs do not fill the SMs the keys are split beyond 512: at least 256 to a single
+// tile's CTA, 128 where there is one tile of rows and the splits are at most 16, 512 to a
+// pair's.  At least 128 / 256 / 512 / 1024, us: 1 query x 1000 keys, 12 over 3 heads 11.0 /
+// 11.9 / 14.3 / 16.5; x 2048, batch 2, 24 over 4 10.7 / 11.8 / 13.7 / 18.9; x 8192, 28 over 4
+// 13.5 / 12.1 / 14.2 / 19.7; 1000 x 1000, 6 heads 19.5 / 17.7 / 18.2 / 18.2; 1 query x 300 keys
+// 9.9 / 9.5 unsplit.
 struct Cut {
   int tiles, splits;
   double us;
@@ -84,8 +92,10 @@ Cut cut(const H3MaskedAttentionArgs& a, const Plan& p, bool pair, int sms) {
   }
   if (a.causal) mean *= 1.0 - 0.5 * (a.q_len < a.k_len ? a.q_len : a.k_len) / (a.k_len > 0 ? a.k_len : 1);
   const bool alone = ctas * c.splits <= sms;   // single tiles with an SM each
-  const auto cta = [&](double b, double block_us) { return 6.0 + block_us * b / c.splits; };
-  const double turns = double(ctas) * c.splits / (alone ? sms : room), block_us = pair ? 2.0 : alone ? 1.3 : 2.1;
+  const bool few = blocks <= 10 * c.splits;
+  const auto cta = [&](double b, double block_us) { return (pair && !few ? 8.5 : 6.0) + block_us * b / c.splits; };
+  const double turns = double(ctas) * c.splits / (alone ? sms : room);
+  const double block_us = pair ? 2.0 : alone ? 1.3 : few ? 2.1 : 2.06;
   if (mean < most) {
     // (a long single tile is alone in the end)
     const double longest = cta(most, pair ? 2.0 : alone ? 1.3 : 1.6), shared = turns * cta(mean, block_us) + 0.1 * longest;

@@ -602,3 +602,30 @@ def test_patched_model_runs_the_provider(device):
             got = patch.wrapper(run, x.clone())
             assert torch.equal(got, want)
             assert "fallback" not in patch.last_report and patch.last_report["counts"]["attention"] == 1
+
+
+@pytest.mark.parametrize("sq,hq,hk,causal,documents,pairs", [
+    (8192, 24, 24, False, 0, 0), (4096, 8, 8, False, 0, 0), (2048, 74, 74, False, 0, 0), (12288, 16, 4, False, 21, 0),
+    (12288, 16, 4, False, 2, 0), (6000, 8, 2, True, 0, 0), (16384, 8, 8, False, 0, 0), (16384, 16, 16, False, 0, 1),
+    (16384, 56, 56, False, 0, 1), (1000, 74, 74, False, 0, 1)])
+def test_the_form_that_measured_shorter(device, sq, hq, hk, causal, documents, pairs):
+    q = torch.empty((1, 1, 1, 128), device=device, dtype=torch.bfloat16)
+    assert plan(q.expand(1, sq, hq, 128), q.expand(1, sq, hk, 128), documents, causal)[0] == pairs
+
+
+@pytest.mark.parametrize("cap,distance", [(0.0, False), (30.0, True)])
+@pytest.mark.parametrize("d,t", [(128, torch.bfloat16), (64, torch.float16)])
+def test_many_single_tiles(device, cap, distance, d, t):
+    """Long inputs whose tiles run singly, two to an SM, with every mask."""
+    n, hq, hk = 1700, 28, 4
+    q, k, v = make(1, n, n, hq, hk, d, t, device)
+    slopes = torch.exp2(-0.1 * torch.arange(1, hq + 1, device=device)) if distance else None
+    more, ref = dict(softcap=cap, slopes=slopes, return_lse=True), dict(scale=d ** -0.5, cap=cap, slopes=slopes)
+    lens = [100, 0, 1, 600, 90, n - 791]
+    offs = [sum(lens[:i]) for i in range(len(lens) + 1)]
+    assert plan(q, k)[0] == 0 and plan(q, k, causal=True)[0] == 0 and plan(q, k, documents=len(lens))[0] == 0
+    check(masked_attention(q, k, v, **more), definition(q, k, v, [(0, 0, n, 0, n)], **ref))
+    check(masked_attention(q, k, v, causal=True, prefix=ints([333], device), **more),
+          definition(q, k, v, [(0, 0, n, 0, n)], causal=True, prefix=[333], **ref))
+    check(masked_attention(q, k, v, q_offsets=ints(offs, device), k_offsets=ints(offs, device), **more),
+          definition(q, k, v, [(0, a, b, a, b) for a, b in zip(offs, offs[1:])], **ref))
