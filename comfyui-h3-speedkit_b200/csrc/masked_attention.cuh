@@ -36,13 +36,13 @@
 // What it runs into: by clocks of a timing copy a step's softmax takes 900 clocks alone
 // and 1300 beside the other stream's, its two products 620 (128 x 64 x 16 reads both
 // operands from shared memory at 54 clocks where 32 would compute it); the exp2 unit
-// (16 a clock and SM) wants 380 of them and the FP32 pipe as many.  Long runs meet the
-// 1000 W cap: the clock falls to 1.6 GHz.  16384 x 16384 tokens, 16 heads of 128: 1850 to
-// 1920 us box to box, 1150 to 1190 TFLOP/s; 8192 x 8192, 24 heads: 713 to 775 us.  Few rows
-// are bound by reading K and V: 1 query, 56 over 8 heads, 32768 keys, batch 2: 50 us, 5.3
-// TB/s.  Tried and slower:
+// (16 a clock and SM) wants 380 of them and the FP32 pipe as many.  Runs of more than a few
+// milliseconds meet the 1000 W cap, and the clock falls to 1.6 GHz: 16384 x 16384 tokens, 16
+// heads of 128, take 1685 us after a pause (1305 TFLOP/s) and 1930 to 2000 in a row; 8192 x
+// 8192, 24 heads 701 and 760 to 800.  Few rows are bound by reading K and V: 1 query, 56 over 8
+// heads, 32768 keys, batch 2: 50 us, 5.4 TB/s.  Tried and slower:
 // S of 128 keys with P over it (the products of a stream wait for its softmax: 2.1 us a
-// block of a pair, now 2.0 and 1.9 in short runs), two threads a row (2.2), P handed on a
+// block of a pair, then 2.0 and 1.9 in short runs), two threads a row (2.2), P handed on a
 // step late, and exponentials before the maximum is known (both 2.0).
 //
 // Every wait is bounded and reports a status code.
@@ -71,10 +71,11 @@ constexpr int kRows = 128;   // query rows per stream (TMEM lanes)
 constexpr int kStep = 64;    // keys per step of a stream
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 enum { kCap = 1, kDistance = 2 };
-// Of eight pairs of exponentials so many take the polynomial.  None / one / two, us: 8192 x
-// 8192 tokens, 24 heads 752 / 714 / 724; 148 tiles of 4096 keys 72 / 71 / 68; 16384 x 16384,
-// 8 heads 1020 / 1010 / 1013 (short of power).  Under a cap, whose tanh wants the same pipe:
-// causal 6000 x 6000, 8 over 2 heads 118 / 123 / 127.
+// Of eight pairs of exponentials so many take the polynomial.  None / one / two, us, after
+// pauses: 16384 x 16384, 16 heads (pairs of tiles) 1797 / 1685 / 1712; 8192 x 8192, 24 heads of
+// 64 600 / 589 / 595; single tiles of 128 channels hardly care: 8192 x 8192, 24 heads 700 / 701 /
+// 706, 16384 x 16384, 8 heads 901 / 904 / 914.  Under a cap, whose tanh wants the same pipe, none:
+// causal 6000 x 6000 with a prefix, 8 over 2 heads 111, with one 123, with two 124.
 constexpr int poly_of_8(int feat) { return feat & kCap ? 0 : 1; }
 constexpr float kGrowth = 8.0f;   // the row maximum may lag this far (in powers of two)
 
@@ -310,8 +311,9 @@ template <typename T, int D, int kFeat>
 struct Softmax {
   static constexpr float kBias = bias_of<T>();
 
-  // The terms of cap R(z), R(y^2) y = tanh(y) for |y| <= 1 (six terms, fitted to 5.9e-7 of
-  // the value, so that small scores under a high cap keep their digits).
+  // The terms of cap R(z), R(y^2) y = tanh(y) for |y| <= 1: six of the least largest relative
+  // error (by Lawson's reweighted least squares), rounded to FP32, 6.1e-7 of the value, so that
+  // small scores under a high cap keep their digits.
   struct Cap {
     uint64_t y, c[6];
     __device__ __forceinline__ explicit Cap(const Args& a) {
@@ -428,7 +430,8 @@ struct Softmax {
       for (int e = 0; e < 4; ++e) m[e] = max3_nan(m[e], __uint_as_float(u[c + 2 * e]), __uint_as_float(u[c + 2 * e + 1]));
   }
   // 2^x of a pair without the exp2 unit: x = n + f with |f| <= 1/2 (the sum with
-  // 1.5 * 2^23 rounds), a polynomial for 2^f (degree 5, fitted to 1.1e-7 relative, 1 at 0)
+  // 1.5 * 2^23 rounds), a polynomial for 2^f (degree 5, 1 at 0, of the least largest relative
+  // error by Lawson's reweighted least squares, rounded to FP32: 1.1e-7)
   // and n added to its exponent.  x <= 16; from -127 down, -inf among it, the result is
   // exactly 0, as a masked key's has to be.  NaN is lost: the caller sees to it.
   static __device__ __forceinline__ void exp2_pair(uint64_t x, float& e0, float& e1) {
@@ -566,7 +569,7 @@ __global__ void __launch_bounds__(Form<kPair>::kThreads, Form<kPair>::kCtas)
   // The CTA's tile, head group, batch and split.  Tiles of one head follow one another
   // and share its keys in L2, unless they differ in work: under a causal mask the
   // heaviest come first, and a long document's tiles of all heads start together (16
-  // over 4 heads, 21 documents in 12288 tokens: 176 us by heads, 172 by tiles).
+  // over 4 heads, 21 documents in 12288 tokens: 176 us by heads, 172 by tiles, then).
   int id = int(blockIdx.x), tile, group, rest;
   const int per_batch = a.groups * a.splits;
   if (a.causal || a.documents) {

@@ -13,8 +13,8 @@
 // CTA computes the sines of its tokens once, for all heads of Q and K.
 //
 // HBM bound: every value of Q and K is read and written once.  16384 tokens, 56 + 56 heads
-// of 128, normalised, 48 pairs turned: 180 us, 5.2 TB/s, 0.80 of a copy's rate (issue slots
-// 64 % busy: the rest is the norm and the rotation between the loads and the stores).  The
+// of 128, normalised, 48 pairs turned: 181 us, 5.2 TB/s, 0.79 of a copy's rate (issue slots
+// 66 % busy: the rest is the norm and the rotation between the loads and the stores).  The
 // table of 98304 tokens, 48 pairs: 15.4 us, where its bytes take 5.9: the rotations'
 // 65 instructions bound it (without the stores still 13.9).  One token: 4.1 us, most of it the launch.
 #include <cuda_bf16.h>
@@ -58,8 +58,10 @@ struct Args {
 };
 
 // (cos, sin) of an angle of `quarter` quarter turns and r more turns, |r| <= 1/8:
-// polynomials in r^2 for sin(2 pi r) / r and cos(2 pi r), fitted to 3.2e-9 and 5.6e-11
-// relative, 1.4e-7 and 8e-8 as FP32 evaluates them.
+// polynomials in r^2 for sin(2 pi r) / r and cos(2 pi r), of the least largest relative error
+// (by Lawson's reweighted least squares, the cosine's 1 at 0 fixed), then rounded to FP32:
+// 4.2e-8 and 8.3e-9 of the value (2 pi in FP32 alone is off by 2.8e-8), 1.4e-7 and 8e-8 as
+// FP32 evaluates them.
 __device__ __forceinline__ float2 cos_sin(int quarter, float r) {
   const float z = r * r;
   float s = fmaf(z, -75.39354705810547f, 81.59235382080078f);
@@ -75,7 +77,9 @@ __device__ __forceinline__ float2 cos_sin(int quarter, float r) {
 }
 
 // A pair's frequency: turns a position, and their fraction as a 64-bit binary one.  Whole
-// positions multiply that and drop whole turns by overflow: exact to 2^-33 turns at 2^31.
+// positions multiply that and drop whole turns by overflow, which loses nothing; what is off is
+// the frequency itself, a rounded double: up to 2^-56 turns at theta^0 / 2 pi = 0.159, so 2^-25
+// turns (1.9e-7 of an angle) at a position of 2^31, as much as FP32 loses in the sine.
 struct Frequency {
   double turns;
   uint64_t fraction;
