@@ -11,7 +11,8 @@ The pairs are numbered axis after axis.  With P pairs in all, pair p is the chan
 (p, P + p) of the head, or (2 p, 2 p + 1) with ``interleaved``; channels from 2 P on
 pass (the partial split-half form of ``ops.qkv``: 96 of 128 channels).  A head's RMS
 norm ``x * weight / sqrt(mean(x^2) + eps)`` may come first.  All in FP32 from the
-stored inputs, rounded once; angles in 64 bits.
+stored inputs (heads whose squares pass its range taken smaller), rounded once; angles in 64
+bits.
 
 ``rope_axes`` rotates Q and K (``inverse=True`` turns back: the transpose, which is
 also the gradient of the rotation); ``rope_table`` makes the BF16 rotation rows that
