@@ -15,7 +15,7 @@
 // HBM bound: every value of Q and K is read and written once.  16384 tokens, 56 + 56 heads
 // of 128, normalised, 48 pairs turned: 181 us, 5.2 TB/s, 0.79 of a copy's rate (issue slots
 // 66 % busy: the rest is the norm and the rotation between the loads and the stores).  The
-// table of 98304 tokens, 48 pairs: 15.4 us, where its bytes take 5.9: the rotations'
+// table of 98304 tokens, 48 pairs: 14.1 to 15.4 us, where its bytes take 5.9: the rotations'
 // 65 instructions bound it (without the stores still 13.9).  One token: 4.1 us, most of it the launch.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

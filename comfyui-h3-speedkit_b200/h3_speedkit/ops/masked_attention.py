@@ -38,7 +38,8 @@ def masked_attention(q, k, v, *, scale=None, softcap=0.0, slopes=None, causal=Fa
     sequence stay as they were in a given ``out`` and ``lse``, and are zero in new
     ones.  Masked values, NaN and infinities among them, reach no result.  Strides are
     multiples of 8 values, operands 16-byte aligned; expanded heads of k and v and
-    expanded batches are taken as they are.
+    expanded batches are taken as they are.  The sum of weights times v is FP32 and is
+    divided at the end: |v| times a row's keys, times 2^8, has to stay below 3.4e38.
 
     Returns out (q's shape and type), or (out, lse) with ``return_lse`` or a given
     ``lse``: FP32 [B, Hq, Sq] ([Hq, Sq] for 3-D operands)."""

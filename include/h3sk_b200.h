@@ -420,7 +420,8 @@ int h3_dense_resources(int* out);
  * strides in values; weight [width] of that type or FP32 (weight_type 2); q dense
  * [rows, width] of `code` (0 INT8, top 127; 1 E4M3, top 448); scale FP32 [rows].
  * width 1..16384, any alignment of the element size (16-byte aligned rows whose
- * width is a multiple of 8 take vector loads).  Returns a cudaError_t.
+ * width is a multiple of 8 take vector loads).  A row whose h, or whose y in FP32, are not
+ * all finite gets a NaN scale.  Returns a cudaError_t.
  */
 int h3_rms_quant_run(const void* x, const void* residual, const void* weight, void* h, void* q, float* scale,
                      int64_t rows, int64_t width, int64_t x_stride, int64_t residual_stride, int64_t h_stride,
@@ -480,7 +481,8 @@ const char* h3_rope_error(int code);
  * [documents or batch]).  A row that sees no key gives zeros and lse -inf (so does
  * one whose visible scores are all -inf); rows of no document, or from q_lengths[b]
  * on, are left as they were, or are written as zeros (lse 0) with fill.  Values in
- * masked places (NaN and infinities among them) reach no result.
+ * masked places (NaN and infinities among them) reach no result.  The weighted sum of V
+ * is FP32 before it is divided: |V| times a row's keys times 2^8 stays below 3.4e38.
  * Strides in values, multiples of 8; 16-byte aligned operands; a stride of 0 shares
  * K and V over heads, and Q, K and V over the batch.  lse is dense [batch, q_heads,
  * q_len] or null.  `workspace` holds h3_masked_attention_workspace(args) bytes
